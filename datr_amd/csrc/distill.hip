@@ -4,7 +4,8 @@
 //   q_v  = softmax over all V columns of z[v] / tau
 //   loss = tau^2 sum_j p_j (log p_j - log q_{i_j}),      d loss / d z_v = tau (q_v - sum over {j : i_j = v} p_j)
 //
-// A row without a valid slot has loss 0 and gradient 0.  Bound by memory: forward reads z once, with the running maximum M
+// A row without a valid slot, or with nothing but -inf in them, has loss 0 and gradient 0; a NaN in a valid slot is the teacher's answer
+// and makes p, the loss and the kept columns' gradient NaN.  Bound by memory: forward reads z once, with the running maximum M
 // and the sum S of exp((z - M) / tau) in fp32; backward reads z again and writes dz, with M, S and the teacher's two from the
 // forward pass.  M and S are kept apart rather than as one log-sum-exp: q = exp((z - M) / tau) / S keeps its relative error
 // for logits of any size.
@@ -47,6 +48,9 @@ __device__ __forceinline__ float teacher_at(int dtype, const void *t, int64_t i)
 struct Soft {
     float m, s;
 };
+
+// whether the teacher's softmax has terms: NaN never raises the maximum, so the sum has to say that one was there
+__device__ __forceinline__ bool kept_any(float m, float s) { return m != -INFINITY || s != 0.f; }
 
 __device__ __forceinline__ float shift(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -107,7 +111,7 @@ __device__ __forceinline__ void finish(bool live, int64_t r, int x, const T *row
         }
     t = join_row<G>(t, c, lds);
     float sum = 0.f;
-    if (live && t.m != -INFINITY) {
+    if (live && kept_any(t.m, t.s)) {
         const float log_s = logf(a.s), log_t = logf(t.s), inv = 1.f / tau;
         for (int j = x; j < sl.k; j += G) {
             const int64_t i = sl.index[r * sl.k + j];
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(TH) void distill_bwd_tiny(const T *__restrict__ z, 
     const int64_t r = (int64_t)blockIdx.x * (TH / G) + threadIdx.x / G;
     if (r >= R) return;
     const float4 st = stats[r];
-    const bool any = st.z != -INFINITY;
+    const bool any = kept_any(st.z, st.w);
     const float g = upstream[r] * tau, inv = 1.f / st.y, t_inv = 1.f / st.w;
     for (int64_t i = threadIdx.x % G; i < V; i += G) {
         float p = 0.f;
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(TH) void distill_bwd(const T *__restrict__ z, int64
     const T *row = z + (live ? r : 0) * ldz;
     T *out = dz + (live ? r : 0) * V;
     const float4 st = stats[live ? r : 0];
-    const bool any = live && st.z != -INFINITY;
+    const bool any = live && kept_any(st.z, st.w);
     const float g = live ? upstream[r] * tau : 0.f, inv = 1.f / st.y;
     const int64_t vectors = V / N, per = (vectors + parts - 1) / parts;
     const int64_t part = G < TH ? 0 : blockIdx.x % parts, lo = part * per, hi = min(lo + per, vectors);

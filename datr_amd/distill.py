@@ -63,9 +63,10 @@ def topk_distillation_loss(student: torch.Tensor, teacher: torch.Tensor, index: 
 
     student [..., V] and teacher [..., k]: float32, float16 or bfloat16; index [..., k] int64 / int32: the student's column
     that each slot stands for.  A slot whose index is outside [0, V) is not valid (rows with fewer kept logits: -1); a row
-    without a valid slot has loss and gradient 0; a column named by several slots takes the sum of their p.  A student's
-    logit of -inf in a column that the teacher kept (p > 0) makes the row's loss infinite, as the formula says, and a row of
-    nothing but -inf has no softmax: NaN.  (The temperature is from 1e-30 to 1e30.)
+    without a valid slot, or with nothing but -inf in its valid slots, has loss and gradient 0; a NaN in a valid slot gives a
+    loss of NaN, and a gradient of NaN in the columns that the row kept; a column named by several slots takes the sum of
+    their p.  A student's logit of -inf in a column that the teacher kept (p > 0) makes the row's loss infinite, as the
+    formula says, and a row of nothing but -inf has no softmax: NaN.  (The temperature is from 1e-30 to 1e30.)
     Differentiable in `student`; the teacher is a constant.  k <= 1024."""
     if student.dtype not in _native.DTYPE or teacher.dtype not in _native.DTYPE:
         name, t = ("student", student) if student.dtype not in _native.DTYPE else ("teacher", teacher)

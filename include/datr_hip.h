@@ -781,7 +781,8 @@ int64_t datr_embedding_backward_workspace_bytes(int64_t tokens, int64_t V, int64
 /* ------------------------------------------------------------------------------------------
  * Distillation from a teacher's top logits, beside the class losses of the teacher-student stage.
  *   loss[r] = tau^2 sum_j p_j (log p_j - log q_{index[r, j]}),  p = softmax(teacher[r] / tau) over the slots whose index is
- *             inside [0, V), q = softmax(z[r] / tau) over all V columns; no such slot: loss 0, gradient 0
+ *             inside [0, V), q = softmax(z[r] / tau) over all V columns; no such slot, or -inf in all of them: loss 0, gradient 0
+ *             (NaN in one of them: loss NaN, dz NaN in the row's kept columns)
  *   dz[r, v] = upstream[r] tau (q_v - sum of p_j over the slots with index[r, j] == v)
  * z [R, V] rows `ldz` elements apart, teacher / index [R, k], k <= 1024, dz [R, V] contiguous, in z's type;
  * stats [R, 4] fp32 (16-byte aligned) carries the softmax statistics from forward to backward; workspace: device memory of
