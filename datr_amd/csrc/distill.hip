@@ -112,13 +112,14 @@ __device__ __forceinline__ void finish(bool live, int64_t r, int x, const T *row
     t = join_row<G>(t, c, lds);
     float sum = 0.f;
     if (live && kept_any(t.m, t.s)) {
-        const float log_s = logf(a.s), log_t = logf(t.s), inv = 1.f / tau;
+        // tau once into the logits' differences and once more into the sum: tau^2 and quotients by tau leave fp32 long before the loss does
+        const float log_s = tau * logf(a.s), log_t = tau * logf(t.s);
         for (int j = x; j < sl.k; j += G) {
             const int64_t i = sl.index[r * sl.k + j];
             if (i < 0 || i >= V) continue;
             const float d = teacher_at(sl.dtype, sl.teacher, r * sl.k + j) - t.m;
             const float p = exp2_fast(d * c) / t.s;
-            if (p != 0.f) sum += p * ((d * inv - log_t) - (((float)row[i] - a.m) * inv - log_s));
+            if (p != 0.f) sum += p * ((d - log_t) - (((float)row[i] - a.m) - log_s));
         }
     }
 #pragma unroll
@@ -131,7 +132,7 @@ __device__ __forceinline__ void finish(bool live, int64_t r, int x, const T *row
             for (int w = 1; w < G / 64; ++w) sum += lds[w].s;
     }
     if (live && x == 0) {
-        loss[r] = tau * tau * sum;
+        loss[r] = tau * sum;
         stats[r] = make_float4(a.m, a.s, t.m, t.s);
     }
 }
@@ -340,6 +341,9 @@ constexpr int kTarget = 512;                        // workgroups of 512 threads
 
 bool sizes_fit(int64_t R, int64_t V, int64_t k) { return R < (V <= 2048 ? 1LL << 25 : 1LL << 22) && V < (1LL << 31) && k <= kMaxSlots; }
 
+// up to where tau^2 log V is an fp32 number
+bool tau_fits(float tau) { return tau >= 1e-30f && tau <= 1e18f; }
+
 }  // namespace
 
 extern "C" {
@@ -353,7 +357,7 @@ int64_t datr_topk_distill_workspace_floats(int dtype, int64_t R, int64_t V) {
 int datr_topk_distill_forward(int dtype, const void *z, int64_t ldz, int teacher_dtype, const void *teacher, const int64_t *index,
                               int64_t R, int64_t V, int64_t k, float tau, float *loss, float *stats, float *workspace,
                               int64_t workspace_floats, void *stream) {
-    if (!elem::known(dtype) || !elem::known(teacher_dtype) || R < 0 || V < 1 || k < 0 || ldz < V || !(tau >= 1e-30f && tau <= 1e30f)) return DATR_EINVAL;
+    if (!elem::known(dtype) || !elem::known(teacher_dtype) || R < 0 || V < 1 || k < 0 || ldz < V || !tau_fits(tau)) return DATR_EINVAL;
     if (R == 0) return DATR_OK;
     if (!sizes_fit(R, V, k)) return DATR_EUNSUPPORTED;
     if (!z || !loss || !stats || !elem::aligned16(stats) || (k > 0 && (!teacher || !index))) return DATR_EINVAL;
@@ -372,7 +376,7 @@ int datr_topk_distill_forward(int dtype, const void *z, int64_t ldz, int teacher
 int datr_topk_distill_backward(int dtype, const void *z, int64_t ldz, int teacher_dtype, const void *teacher, const int64_t *index,
                                int64_t R, int64_t V, int64_t k, float tau, const float *stats, const float *upstream, void *dz,
                                void *stream) {
-    if (!elem::known(dtype) || !elem::known(teacher_dtype) || R < 0 || V < 1 || k < 0 || ldz < V || !(tau >= 1e-30f && tau <= 1e30f)) return DATR_EINVAL;
+    if (!elem::known(dtype) || !elem::known(teacher_dtype) || R < 0 || V < 1 || k < 0 || ldz < V || !tau_fits(tau)) return DATR_EINVAL;
     if (R == 0) return DATR_OK;
     if (!sizes_fit(R, V, k)) return DATR_EUNSUPPORTED;
     if (!z || !stats || !elem::aligned16(stats) || !upstream || !dz || (k > 0 && (!teacher || !index))) return DATR_EINVAL;

@@ -66,7 +66,8 @@ def topk_distillation_loss(student: torch.Tensor, teacher: torch.Tensor, index: 
     without a valid slot, or with nothing but -inf in its valid slots, has loss and gradient 0; a NaN in a valid slot gives a
     loss of NaN, and a gradient of NaN in the columns that the row kept; a column named by several slots takes the sum of
     their p.  A student's logit of -inf in a column that the teacher kept (p > 0) makes the row's loss infinite, as the
-    formula says, and a row of nothing but -inf has no softmax: NaN.  (The temperature is from 1e-30 to 1e30.)
+    formula says, and a row of nothing but -inf has no softmax: NaN.  The temperature is from 1e-30 to 1e18; it
+    scales, squared, the roundings of the softmaxes' 32-bit sums and logarithms too, which a large one leaves little beside.
     Differentiable in `student`; the teacher is a constant.  k <= 1024."""
     if student.dtype not in _native.DTYPE or teacher.dtype not in _native.DTYPE:
         name, t = ("student", student) if student.dtype not in _native.DTYPE else ("teacher", teacher)
@@ -83,8 +84,8 @@ def topk_distillation_loss(student: torch.Tensor, teacher: torch.Tensor, index: 
     if k > MAX_SLOTS:
         raise NotImplementedError(f"topk_distillation_loss: at most {MAX_SLOTS} kept logits a row, got {k}")
     tau = float(temperature)
-    if not 1e-30 <= tau <= 1e30:
-        raise ValueError(f"topk_distillation_loss: a temperature from 1e-30 to 1e30, got {temperature}")
+    if not 1e-30 <= tau <= 1e18:
+        raise ValueError(f"topk_distillation_loss: a temperature from 1e-30 to 1e18, got {temperature}")
     if not student.is_cuda:
         raise RuntimeError("topk_distillation_loss: Not implemented on the CPU")
     device = student.device

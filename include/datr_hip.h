@@ -787,7 +787,7 @@ int64_t datr_embedding_backward_workspace_bytes(int64_t tokens, int64_t V, int64
  * z [R, V] rows `ldz` elements apart, teacher / index [R, k], k <= 1024, dz [R, V] contiguous, in z's type;
  * stats [R, 4] fp32 (16-byte aligned) carries the softmax statistics from forward to backward; workspace: device memory of
  * datr_topk_distill_workspace_floats(dtype, R, V) floats (may be 0), the call's own while it runs.
- * R < 2^22 (2^25 for V <= 2048), tau from 1e-30 to 1e30.
+ * R < 2^22 (2^25 for V <= 2048), tau from 1e-30 to 1e18.
  * ------------------------------------------------------------------------------------------ */
 int datr_topk_distill_forward(int dtype, const void *z, int64_t ldz, int teacher_dtype, const void *teacher,
                               const int64_t *index, int64_t R, int64_t V, int64_t k, float tau, float *loss,
