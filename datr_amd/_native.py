@@ -10,6 +10,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # DATR_HIP_LIB points at an alternative build of the same ABI (e.g. the -DDATR_PROBE build used
@@ -222,6 +223,11 @@ def on_device(device):
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def carries_tangent(t: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation has a tangent for `t` (such a tensor need not require a gradient)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def current_stream_ptr(device: torch.device) -> int:

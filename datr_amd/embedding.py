@@ -7,12 +7,12 @@
 
 Tables are float32, float16 or bfloat16 device tensors.  The gradient adds a row's tokens in ascending order in 32 bits and
 rounds once: it does not depend on the launch, where atomics would.  An id outside [0, rows) gives a row of zeros and no
-gradient (no host synchronisation to look for one)."""
+gradient (no host synchronisation to look for one).  Both directions are linear and each is the other's derivative, so they
+differentiate any number of times, in reverse and in forward mode."""
 from __future__ import annotations
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -65,9 +65,15 @@ def embedding_backward(ids: torch.Tensor, upstream: torch.Tensor, rows: int, sca
     pad = _padding(padding_idx, rows)
     if not upstream.is_cuda:
         raise RuntimeError("embedding_backward: Not implemented on the CPU")
-    device = upstream.device
-    if ids.device != device:
+    if ids.device != upstream.device:
         raise ValueError("embedding_backward: ids and upstream are on different devices")
+    if (upstream.requires_grad and torch.is_grad_enabled()) or _native.carries_tangent(upstream):
+        return _EmbeddingGradient.apply(ids, upstream, rows, float(scale), pad)
+    return _backward(ids, upstream, rows, scale, pad)
+
+
+def _backward(ids: torch.Tensor, upstream: torch.Tensor, rows: int, scale: float, pad: int) -> torch.Tensor:
+    shape, device = upstream.shape, upstream.device
     D, flat = shape[-1], _ids64(ids)
     tokens = flat.numel()
     up = upstream if len(shape) == 2 else upstream.reshape(tokens, D)
@@ -89,14 +95,42 @@ class _Embedding(Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
         return _forward(ids, table, scale)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, upstream):
         ids, = ctx.saved_tensors
         return None, embedding_backward(ids, upstream, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+
+    @staticmethod
+    def jvp(ctx, _ids, table, _scale, _padding_idx):
+        ids, = ctx.saved_tensors
+        return embedding(ids, table, ctx.scale, ctx.padding_idx)
+
+
+class _EmbeddingGradient(Function):
+    """embedding_backward as a node of its own, for derivatives of the gradient; `pad` is -1 without a padding row."""
+
+    @staticmethod
+    def forward(ctx, ids, upstream, rows, scale, pad):
+        ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
+        ctx.rows, ctx.scale, ctx.pad = rows, scale, pad
+        return _backward(ids, upstream, rows, scale, pad)
+
+    @staticmethod
+    def backward(ctx, along):
+        ids, = ctx.saved_tensors
+        if ctx.pad >= 0:                                   # the padding row's tokens took no part
+            ids = torch.where(ids == ctx.pad, -1, ids)
+        return None, embedding(ids, along, ctx.scale), None, None, None
+
+    @staticmethod
+    def jvp(ctx, _ids, upstream, _rows, _scale, _pad):
+        ids, = ctx.saved_tensors
+        return embedding_backward(ids, upstream, ctx.rows, ctx.scale, None if ctx.pad < 0 else ctx.pad)
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx=None) -> torch.Tensor:
@@ -112,14 +146,15 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
         raise RuntimeError("embedding: Not implemented on the CPU")
     if ids.device != table.device:
         raise ValueError("embedding: ids and table are on different devices")
-    if torch.is_grad_enabled() and table.requires_grad:
+    if (table.requires_grad and torch.is_grad_enabled()) or _native.carries_tangent(table):
         return _Embedding.apply(ids, table, float(scale), padding_idx)
     return _forward(ids, table, float(scale))
 
 
 class FastEmbedding(torch.nn.Embedding):
     """nn.Embedding (same parameters, same state_dict keys) with a scale, on the kernels above for device tables; host tables
-    and nn.Embedding's max_norm / scale_grad_by_freq / sparse take its own path."""
+    and nn.Embedding's max_norm / scale_grad_by_freq / sparse take its own path, and so does a call below a function transform
+    (torch.func)."""
 
     def __init__(self, *args, scale: float = 1.0, **kw):
         super().__init__(*args, **kw)
@@ -127,7 +162,7 @@ class FastEmbedding(torch.nn.Embedding):
 
     def forward(self, ids):
         if (self.weight.is_cuda and self.weight.dtype in _native.DTYPE and self.max_norm is None and not self.scale_grad_by_freq
-                and not self.sparse):
+                and not self.sparse and not torch._C._are_functorch_transforms_active()):
             return embedding(ids, self.weight, self.scale, self.padding_idx)
         y = super().forward(ids)
         return y if self.scale == 1.0 else y * self.scale
