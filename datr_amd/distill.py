@@ -68,7 +68,7 @@ def topk_distillation_loss(student: torch.Tensor, teacher: torch.Tensor, index: 
     their p.  A student's logit of -inf in a column that the teacher kept (p > 0) makes the row's loss infinite, as the
     formula says, and a row of nothing but -inf has no softmax: NaN.  The temperature is from 1e-30 to 1e18; it
     scales, squared, the roundings of the softmaxes' 32-bit sums and logarithms too, which a large one leaves little beside.
-    Differentiable in `student`; the teacher is a constant.  k <= 1024."""
+    Differentiable in `student`, once and in reverse mode; the teacher is a constant.  k <= 1024."""
     if student.dtype not in _native.DTYPE or teacher.dtype not in _native.DTYPE:
         name, t = ("student", student) if student.dtype not in _native.DTYPE else ("teacher", teacher)
         raise TypeError(f"topk_distillation_loss: {name} is float32, float16 or bfloat16, got {t.dtype}")
@@ -86,6 +86,8 @@ def topk_distillation_loss(student: torch.Tensor, teacher: torch.Tensor, index: 
     tau = float(temperature)
     if not 1e-30 <= tau <= 1e18:
         raise ValueError(f"topk_distillation_loss: a temperature from 1e-30 to 1e18, got {temperature}")
+    if _native.carries_tangent(student):
+        raise RuntimeError("topk_distillation_loss has no forward-mode derivative")
     if not student.is_cuda:
         raise RuntimeError("topk_distillation_loss: Not implemented on the CPU")
     device = student.device

@@ -45,9 +45,9 @@ def _quantize(x2: torch.Tensor):
 
 
 def quantize_rows(x: torch.Tensor):
-    """x [..., K] -> (q int8 [..., K], scale float32 [...]) with x ~ q * scale[..., None]: scale = max|x| / 127 over the row.
-    A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN (and q 0).  q's rows are held at a distance of
-    whole 128-byte lines, the layout that `linear_int8` reads without a copy."""
+    """x [..., K] -> (q int8 [..., K], scale float32 [...]) with x ~ q * scale[..., None]: scale = max|x| / 127 over the row; x is
+    taken as a constant.  A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN (and q 0).  q's rows are held
+    at a distance of whole 128-byte lines, the layout that `linear_int8` reads without a copy."""
     _check_float(x, "quantize_rows")
     if not x.is_cuda:
         raise RuntimeError("quantize_rows: Not implemented on the CPU")
@@ -78,6 +78,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError(f"linear_int8: weight_scale and bias have {N} entries")
     if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad(), or detach its inputs")
+    if _native.carries_tangent(x) or _native.carries_tangent(weight_scale) or (bias is not None and _native.carries_tangent(bias)):
+        raise RuntimeError("linear_int8 has no gradient, in forward mode either")
     if not x.is_cuda:
         raise RuntimeError("linear_int8: Not implemented on the CPU")
     device = x.device
