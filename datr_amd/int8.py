@@ -118,6 +118,17 @@ class Int8Linear(torch.nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float().clone())
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        weight, scale = state_dict.get(prefix + "weight"), state_dict.get(prefix + "weight_scale")
+        if weight is not None and weight.dtype is not torch.int8:
+            # a cast would leave zeros; an error stops the load whatever `strict` says
+            error_msgs.append(f"{prefix}weight is int8 with a scale per row, got {weight.dtype}: load a float checkpoint before the layer "
+                              "is quantised")
+        elif (weight is None) != (scale is None):
+            error_msgs.append(f"{prefix}weight and {prefix}weight_scale belong together, got one of them")
+        else:
+            super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
     def forward(self, x: torch.Tensor, relu: bool = False) -> torch.Tensor:
         if self.weight.stride(0) % 16:
             # a move to another device packs the rows: lay them out again, once, instead of copying them on every call
