@@ -38,6 +38,11 @@ def load_model_state(model: torch.nn.Module, checkpoint, key: Optional[str] = No
     if ignore:
         sd = OrderedDict((k, v) for k, v in sd.items() if not any(w in k for w in ignore))
         strict = False
+    own = model.state_dict()
+    for k, v in sd.items():
+        # an 8-bit layer's integers (datr_amd.int8) in a float layer: a copy would cast them without their scales
+        if isinstance(v, torch.Tensor) and v.dtype is torch.int8 and k in own and own[k].dtype.is_floating_point:
+            raise RuntimeError(f"load_model_state: {k} is int8 in the checkpoint and {own[k].dtype} in the model: quantise the model first")
     return model.load_state_dict(sd, strict=strict)
 
 

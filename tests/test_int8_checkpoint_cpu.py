@@ -39,3 +39,17 @@ def test_integers_and_scales_are_loaded_together(monkeypatch):
     assert same(b.state_dict(), a.state_dict())
     with pytest.raises(RuntimeError, match="size mismatch"):
         host_layer(monkeypatch, 50, 34).load_state_dict(b.state_dict())
+
+
+@pytest.mark.parametrize("ignore", [[], ["label_enc"]])
+def test_a_checkpoint_of_integers_is_no_float_layers(monkeypatch, ignore):
+    torch.manual_seed(2)
+    model = torch.nn.Sequential(torch.nn.Linear(50, 33))
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    integers = torch.nn.Sequential(host_layer(monkeypatch, 50, 33)).state_dict()
+    with pytest.raises(RuntimeError, match="0.weight is int8"):
+        load_model_state(model, {"model": integers}, ignore_keywords=ignore)
+    assert same(before, model.state_dict())
+    model[0] = host_layer(monkeypatch, 50, 33)
+    load_model_state(model, {"model": integers}, ignore_keywords=ignore)
+    assert same(integers, torch.nn.Sequential(model[0]).state_dict())
