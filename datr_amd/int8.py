@@ -128,12 +128,22 @@ class Int8Linear(torch.nn.Module):
             error_msgs.append(f"{prefix}weight and {prefix}weight_scale belong together, got one of them")
         else:
             super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+            self._hold_rows()
 
-    def forward(self, x: torch.Tensor, relu: bool = False) -> torch.Tensor:
-        if self.weight.stride(0) % 16:
-            # a move to another device packs the rows: lay them out again, once, instead of copying them on every call
+    def _hold_rows(self) -> None:
+        """Rows at 16-byte borders: a move to another device and an assigned checkpoint pack them, and linear_int8 would copy them
+        on every call.  Not in forward: a buffer bound anew inside a graph's capture, on one of two streams or under inference
+        mode is not what the next call may use."""
+        if self.weight.stride(0) % 16 or self.weight.stride(1) != 1:
             held = torch.empty((self.out_features, -(-self.in_features // 16) * 16), dtype=torch.int8, device=self.weight.device)
             self.weight = held[:, :self.in_features].copy_(self.weight)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._hold_rows()
+        return self
+
+    def forward(self, x: torch.Tensor, relu: bool = False) -> torch.Tensor:
         return linear_int8(x, self.weight, self.weight_scale, self.bias, relu=relu)
 
     def extra_repr(self) -> str:
