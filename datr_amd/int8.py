@@ -108,7 +108,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
 
 class Int8Linear(torch.nn.Module):
-    """An nn.Linear's weights as int8 with one scale per output channel; no parameters, no gradient."""
+    """An nn.Linear's weights as int8 with one scale per output channel; no parameters, no gradient.  The scales and the bias are
+    float32 and stay so when the model is cast; the result has x's type."""
 
     def __init__(self, linear: torch.nn.Linear):
         super().__init__()
@@ -129,6 +130,7 @@ class Int8Linear(torch.nn.Module):
         else:
             super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
             self._hold_rows()
+            self._keep_float32(self.weight_scale, self.bias)              # (assigned from a checkpoint in half precision)
 
     def _hold_rows(self) -> None:
         """Rows at 16-byte borders: a move to another device and an assigned checkpoint pack them, and linear_int8 would copy them
@@ -138,9 +140,18 @@ class Int8Linear(torch.nn.Module):
             held = torch.empty((self.out_features, -(-self.in_features // 16) * 16), dtype=torch.int8, device=self.weight.device)
             self.weight = held[:, :self.in_features].copy_(self.weight)
 
+    def _keep_float32(self, scale, bias) -> None:
+        # half() and its like cast a model's float buffers; the layer reads these two in 32 bits whatever x is
+        for name, before in (("weight_scale", scale), ("bias", bias)):
+            now = getattr(self, name)
+            if now is not None and now.dtype is not torch.float32:
+                setattr(self, name, before.to(now.device, torch.float32))
+
     def _apply(self, fn, recurse=True):
+        scale, bias = self.weight_scale, self.bias
         super()._apply(fn, recurse)
         self._hold_rows()
+        self._keep_float32(scale, bias)
         return self
 
     def forward(self, x: torch.Tensor, relu: bool = False) -> torch.Tensor:
