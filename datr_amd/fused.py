@@ -9,6 +9,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _native
+from .int8 import Int8Linear
 
 # The kernels behind these nodes read raw float32 pointers.  Under torch.autocast (engine.py runs the
 # model under it when args.amp is set, /root/reference/engine.py:59) a torch.mm / addmm INSIDE a
@@ -291,10 +292,9 @@ def ffn_relu(x: torch.Tensor, linear1: torch.nn.Linear, linear2: torch.nn.Linear
     """linear2(relu(linear1(x))).  Device float32 tensors take the fused path above; anything
     else evaluates the reference's own op sequence
     (/root/reference/models/dino/deformable_transformer.py:803-806)."""
-    from .int8 import Int8Linear
     if isinstance(linear1, Int8Linear):                    # the ReLU in the integer product's epilogue
         return linear2(linear1(x, relu=True))
-    if x.is_cuda and x.dtype == torch.float32 and linear1.bias is not None \
+    if x.is_cuda and x.dtype == torch.float32 and not isinstance(linear2, Int8Linear) and linear1.bias is not None \
             and linear2.bias is not None and linear1.out_features % 4 == 0:
         return _FFNRelu.apply(x, linear1.weight, linear1.bias, linear2.weight, linear2.bias)
     return linear2(torch.relu(linear1(x)))
