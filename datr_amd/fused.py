@@ -458,7 +458,7 @@ def ffn_add_norm(x: torch.Tensor, linear1: torch.nn.Linear, linear2: torch.nn.Li
     three handles (output + next_pos, output, output) -- query, value input, residual -- and sums their gradients
     while it loads them, where `q = src + pos` and the three-way gradient sum each cost passes over the tokens."""
     if not (x.is_cuda and x.dtype == torch.float32 and x.shape[-1] == 256
-            and isinstance(linear1, torch.nn.Linear) and isinstance(linear2, torch.nn.Linear) and linear1.bias is not None
+            and not isinstance(linear1, Int8Linear) and not isinstance(linear2, Int8Linear) and linear1.bias is not None
             and linear2.bias is not None and linear1.out_features % 4 == 0 and linear2.out_features == 256
             and norm.elementwise_affine and norm.bias is not None and tuple(norm.normalized_shape) == (256,)
             and torch.is_grad_enabled()):
