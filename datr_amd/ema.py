@@ -71,9 +71,12 @@ def _ema_update_(ema_model: nn.Module, model: nn.Module, d: float) -> None:
     device that is ONE launch of csrc/ema.hip over all float32 tensors (tables cached per EMA model
     and rebuilt when a storage moved); tensors on the host (CPU runs) take the same arithmetic
     through torch._foreach."""
-    msd = _unwrap(model).state_dict()
+    msd, esd = _unwrap(model).state_dict(), ema_model.state_dict()
     first, count = {}, {}
-    for k, v in ema_model.state_dict().items():
+    for k, v in esd.items():
+        if any(k + "_scale" in sd and k in sd and sd[k].dtype is torch.int8 for sd in (esd, msd)):
+            raise RuntimeError(f"EMA update: {k} belongs to an 8-bit layer, whose integers and scales have no average; keep the teacher in "
+                               "floats and quantise a copy of it after the update (datr_amd.int8.quantize_ffn_)")
         if v.dtype.is_floating_point:
             ptr = v.data_ptr()
             if ptr not in first:

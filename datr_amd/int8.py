@@ -164,7 +164,10 @@ class Int8Linear(torch.nn.Module):
 def quantize_ffn_(module: torch.nn.Module) -> int:
     """Replaces `linear1` and `linear2` of every encoder / decoder layer below `module` (an evaluation model or a frozen
     teacher on its device) by Int8Linear, in place; returns how many layers were changed.  The rest of the model keeps its
-    precision: the feed-forward products are over half of a forward pass' matrix work."""
+    precision: the feed-forward products are over half of a forward pass' matrix work.
+
+    A teacher that takes EMA updates stays in floats: datr_amd.ema refuses 8-bit layers, so quantise a deepcopy of it after
+    each update."""
     changed = 0
     for layer in list(module.modules()):
         pair = [getattr(layer, name, None) for name in ("linear1", "linear2")]
