@@ -59,6 +59,10 @@ def prepare_for_cdn(dn_args, training, num_queries, num_classes, hidden_dim, lab
             chosen = torch.nonzero(p < (label_noise_ratio * 0.5)).view(-1)
             noised_labels.scatter_(0, chosen, noise["new_label"].to(device))
         else:
+            if num_classes > label_enc.weight.shape[0]:
+                # on the device an id outside the table raises nothing (a row of zeros)
+                raise ValueError(f"prepare_for_cdn: labels are drawn from {num_classes} classes, the label table has "
+                                 f"{label_enc.weight.shape[0]} rows (dn_labelbook_size + 1)")
             # same distribution as dn_components.py:60-63 (flip each label with probability
             # ratio/2 to a uniform class) without `nonzero`, whose data-dependent size costs a
             # device->host sync; the random stream is not the reference's either way
