@@ -180,9 +180,26 @@ struct Product {
     int relu;
 };
 
+// The sum meets the token's scale first and the channel's in one fused operation with the bias: the two scales' product by itself may
+// leave fp32 where the result does not.  |sum| < 2^31, so a token scale up to 2^96 keeps the first product finite; a larger one
+// (at most 2^121.02) gives 2^25 to the channel's scale, which stays finite for a sum of 0's sake.
+constexpr float kLargeScale = 0x1p96f, kGive = 0x1p25f, kFinite = 0x1.fffffep127f;
+
+__device__ __forceinline__ float token_part(float s) { return s > kLargeScale ? s * (1.f / kGive) : s; }
+__device__ __forceinline__ float channel_part_large(float ws) {
+    return fabsf(ws) <= kFinite ? fminf(fmaxf(ws * kGive, -kFinite), kFinite) : ws;
+}
+
+// s and ws: the parts above
 __device__ __forceinline__ float finish(const Product &p, int acc, float s, float ws, float b) {
-    const float v = (float)acc * (s * ws) + b;
+    const float v = (float)acc * s * ws + b;
     return p.relu && v < 0.f ? 0.f : v;                          // a NaN stays one
+}
+
+// one result of a row whose scale is s
+__device__ __forceinline__ float finish_one(const Product &p, int acc, float s, int64_t n) {
+    const float ws = p.w_scale[n];
+    return finish(p, acc, token_part(s), s > kLargeScale ? channel_part_large(ws) : ws, p.bias ? p.bias[n] : 0.f);
 }
 
 // rows from row0 on, as a buffer whose range check gives zeros behind the last row's K columns (rounded up to a word)
@@ -235,12 +252,14 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_tile(Product p, int tiles_n
     };
 
     const int wn = wave % WN, wm = wave / WN;
-    // the channels' scales and biases wait behind the operands' LDS, the tokens' scales in registers
+    // the channels' scales, biases and scales for tokens of a large one wait behind the operands' LDS, the tokens' scales in registers
     constexpr unsigned SCALES = S * STAGE;
     for (int c = threadIdx.x; c < BN; c += 64 * WAVES) {
         const bool in = n0 + c < p.N;
-        *reinterpret_cast<lds_float *>((uintptr_t)(SCALES + c * 4u)) = in ? p.w_scale[n0 + c] : 0.f;
+        const float ws = in ? p.w_scale[n0 + c] : 0.f;
+        *reinterpret_cast<lds_float *>((uintptr_t)(SCALES + c * 4u)) = ws;
         *reinterpret_cast<lds_float *>((uintptr_t)(SCALES + (BN + c) * 4u)) = in && p.bias ? p.bias[n0 + c] : 0.f;
+        *reinterpret_cast<lds_float *>((uintptr_t)(SCALES + (2 * BN + c) * 4u)) = channel_part_large(ws);
     }
     float token_scale[TM];
 #pragma unroll
@@ -283,13 +302,14 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_tile(Product p, int tiles_n
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
         const int64_t m_first = m0 + (wm * TM + j) * 32;
-        const float s = token_scale[j];
+        const float s = token_part(token_scale[j]);
+        const unsigned scales = SCALES + (token_scale[j] > kLargeScale ? 2 * BN * 4u : 0u);
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = i * 32 + 8 * g + 4 * half;
-                const f32x4 ws = *reinterpret_cast<const lds_f32x4 *>((uintptr_t)(SCALES + (wn * TN * 32 + c) * 4u));
+                const f32x4 ws = *reinterpret_cast<const lds_f32x4 *>((uintptr_t)(scales + (wn * TN * 32 + c) * 4u));
                 const f32x4 bias = *reinterpret_cast<const lds_f32x4 *>((uintptr_t)(SCALES + (BN + wn * TN * 32 + c) * 4u));
                 T out[4];
 #pragma unroll
@@ -391,7 +411,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gemm_few(Product p) {
         const float s = p.a_scale[m];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) ((T *)p.y)[m * p.ldy + n + e] = (T)finish(p, sum[e], s, p.w_scale[n + e], p.bias ? p.bias[n + e] : 0.f);
+            if (n + e < p.N) ((T *)p.y)[m * p.ldy + n + e] = (T)finish_one(p, sum[e], s, n + e);
     }
 }
 
@@ -472,7 +492,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gemm_one(Product p, const X *_
     const int64_t n = n0 + (lane >> 4) * 4;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) ((T *)p.y)[n + e] = (T)finish(p, sum[e], rs.scale(), p.w_scale[n + e], p.bias ? p.bias[n + e] : 0.f);
+        if (n + e < p.N) ((T *)p.y)[n + e] = (T)finish_one(p, sum[e], rs.scale(), n + e);
 }
 
 template <class T, int TN, int TM, int WN, int WM, int S>
@@ -480,7 +500,7 @@ int launch_tile(const Product &p, hipStream_t st) {
     constexpr int BN = 32 * TN * WN, BM = 32 * TM * WM;
     const int64_t tn = (p.N + BN - 1) / BN, tm = (p.M + BM - 1) / BM;
     if (tn * tm * 64 * WN * WM >= (1LL << 32)) return DATR_EUNSUPPORTED;
-    constexpr int lds = S * (BN + BM) * kRowBytes + BN * 8;
+    constexpr int lds = S * (BN + BM) * kRowBytes + BN * 12;
     auto kernel = gemm_tile<T, TN, TM, WN, WM, S>;
     if (lds > 65536 && hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return DATR_ELAUNCH;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tn * tm)), dim3(64 * WN * WM), lds, st, p, (int)tn, (int)tm);
