@@ -12,7 +12,7 @@ differentiate any number of times, in reverse and in forward mode."""
 from __future__ import annotations
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import _native
 
@@ -67,9 +67,7 @@ def embedding_backward(ids: torch.Tensor, upstream: torch.Tensor, rows: int, sca
         raise RuntimeError("embedding_backward: Not implemented on the CPU")
     if ids.device != upstream.device:
         raise ValueError("embedding_backward: ids and upstream are on different devices")
-    if (upstream.requires_grad and torch.is_grad_enabled()) or _native.carries_tangent(upstream):
-        return _EmbeddingGradient.apply(ids, upstream, rows, float(scale), pad)
-    return _backward(ids, upstream, rows, scale, pad)
+    return _gradient(ids, upstream, rows, float(scale), pad)
 
 
 def _backward(ids: torch.Tensor, upstream: torch.Tensor, rows: int, scale: float, pad: int) -> torch.Tensor:
@@ -91,46 +89,54 @@ def _backward(ids: torch.Tensor, upstream: torch.Tensor, rows: int, scale: float
     return grad
 
 
+def _gradient(ids: torch.Tensor, upstream: torch.Tensor, rows: int, scale: float, pad: int) -> torch.Tensor:
+    if (upstream.requires_grad and torch.is_grad_enabled()) or _native.carries_tangent(upstream):
+        return _EmbeddingGradient.apply(ids, upstream, rows, scale, pad)
+    return _backward(ids, upstream, rows, scale, pad)
+
+
 class _Embedding(Function):
+    """`pad` is -1 without a padding row."""
+
     @staticmethod
-    def forward(ctx, ids, table, scale, padding_idx):
+    def forward(ctx, ids, table, scale, pad):
         ctx.save_for_backward(ids)
-        ctx.save_for_forward(ids)
-        ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(ids)
+        ctx.rest = table.shape[0], scale, pad
         return _forward(ids, table, scale)
 
     @staticmethod
     def backward(ctx, upstream):
-        ids, = ctx.saved_tensors
-        return None, embedding_backward(ids, upstream, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+        return None, _gradient(*ctx.saved_tensors, upstream, *ctx.rest), None, None
 
     @staticmethod
-    def jvp(ctx, _ids, table, _scale, _padding_idx):
+    def jvp(ctx, _ids, table, _scale, _pad):
         ids, = ctx.saved_tensors
-        return embedding(ids, table, ctx.scale, ctx.padding_idx)
+        return embedding(ids, table, ctx.rest[1])
 
 
 class _EmbeddingGradient(Function):
-    """embedding_backward as a node of its own, for derivatives of the gradient; `pad` is -1 without a padding row."""
+    """embedding_backward as a node of its own, for derivatives of the gradient."""
 
     @staticmethod
     def forward(ctx, ids, upstream, rows, scale, pad):
         ctx.save_for_backward(ids)
         ctx.save_for_forward(ids)
-        ctx.rows, ctx.scale, ctx.pad = rows, scale, pad
+        ctx.rest = rows, scale, pad
         return _backward(ids, upstream, rows, scale, pad)
 
     @staticmethod
     def backward(ctx, along):
         ids, = ctx.saved_tensors
-        if ctx.pad >= 0:                                   # the padding row's tokens took no part
-            ids = torch.where(ids == ctx.pad, -1, ids)
-        return None, embedding(ids, along, ctx.scale), None, None, None
+        _, scale, pad = ctx.rest
+        if pad >= 0:                                       # the padding row's tokens took no part
+            ids = torch.where(ids == pad, -1, ids)
+        return None, embedding(ids, along, scale), None, None, None
 
     @staticmethod
     def jvp(ctx, _ids, upstream, _rows, _scale, _pad):
-        ids, = ctx.saved_tensors
-        return embedding_backward(ids, upstream, ctx.rows, ctx.scale, None if ctx.pad < 0 else ctx.pad)
+        return _gradient(*ctx.saved_tensors, upstream, *ctx.rest)
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx=None) -> torch.Tensor:
@@ -141,13 +147,13 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
         raise ValueError(f"embedding: the table is [rows, width], got {tuple(table.shape)}")
     if table.dtype not in _native.DTYPE:
         raise TypeError(f"embedding: float32, float16 or bfloat16 tables, got {table.dtype}")
-    _padding(padding_idx, table.shape[0])
+    pad = _padding(padding_idx, table.shape[0])
     if not table.is_cuda:
         raise RuntimeError("embedding: Not implemented on the CPU")
     if ids.device != table.device:
         raise ValueError("embedding: ids and table are on different devices")
     if (table.requires_grad and torch.is_grad_enabled()) or _native.carries_tangent(table):
-        return _Embedding.apply(ids, table, float(scale), padding_idx)
+        return _Embedding.apply(ids, table, float(scale), pad)
     return _forward(ids, table, float(scale))
 
 
