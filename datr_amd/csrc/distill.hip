@@ -28,7 +28,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //   and R >= 1024
 //   else          a workgroup, and several where few rows would leave the chip idle: forward parts are joined by a second
 //                 launch, backward parts need no join.  4096 rows of 128 000 bf16: 585 us for both passes over 3.15 GB = 5.4 TB/s;
-//                 1000 rows of 50 257 fp32: 108 us = 5.6 TB/s (a large copy on this card: 4.8).  dz goes out by streaming stores:
+//                 1000 rows of 50 257 fp32: 108 us = 5.6 TB/s (a large copy on this card: 4.7).  dz goes out by streaming stores:
 //                 kept in the caches it costs 25 % more at 1000 x 50 257, where z would still be there for backward
 constexpr int kGroupThreads = 256;
 constexpr int kRowThreads = 512;

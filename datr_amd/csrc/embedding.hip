@@ -7,8 +7,8 @@
 // Both are bound by memory: forward reads min(T, V) rows and writes T, backward reads T rows of dy and writes all V rows
 // of dW.  No atomics: every row of dW has one owner that adds its tokens in ascending order.
 //
-// 32 768 tokens of 128 000 rows x 4096 bf16: 355 us for both directions over 1.85 GB = 5.2 TB/s (a large copy on this card: 4.8) --
-// forward 94, zeros beside the sort 175, sums 82, their join 9.
+// 32 768 tokens of 128 000 rows x 4096 bf16: 356 us for both directions over 1.85 GB = 5.2 TB/s (a large copy on this card: 4.7).  In
+// a kernel trace, which adds a little to each: forward 93, the sort with the zeros beside it 175, sums 82, their join 9.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

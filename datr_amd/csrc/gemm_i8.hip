@@ -1,12 +1,12 @@
 // gemm_i8.hip -- a linear layer in 8-bit integers with one scale for each token and one for each output channel (gfx950).
 //
 //   s_m    = max_k |x[m, k]| / 127,       q[m, k] = x[m, k] / s_m rounded to nearest, ties to even
-//   y[m,n] = relu?( s_m w_n * sum_k q[m, k] W[n, k] + bias[n] )          W int8 [N, K] with scales w_n, sums in 32-bit integers
+//   y[m,n] = relu?( sum_k q[m, k] W[n, k] * s_m * w_n + bias[n] )          W int8 [N, K] with scales w_n, sums in 32-bit integers
 //
 // The integer sum is exact (|sum| <= 127 * 128 * K < 2^31 for K <= 131072), so y does not depend on tiles or on the order of sums.
 //
-// Two launches (one for a single token): the rows of x are quantised (bound by memory: x once, q once; 88 892 x 2048 fp32: 140 us =
-// 6.3 TB/s), then multiplied.  The product's W is the matrix instruction's first operand: a lane then holds four consecutive
+// Two launches (one for a single token): the rows of x are quantised (bound by memory: x once, q once; 88 892 x 2048 fp32: 147 us on
+// average, 136 at best = 6.2 and 6.7 TB/s), then multiplied.  The product's W is the matrix instruction's first operand: a lane then holds four consecutive
 // channels of one token, which leave as one 8- or 16-byte piece.
 #include <hip/hip_runtime.h>
 
@@ -214,8 +214,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const int8_t *base, in
 // place c ^ ((r >> 1) & 7) -- by permuting the source addresses, the LDS side being lane-linear -- so that a fragment's
 // ds_read_b128 meets every bank once.
 //
-// 8192 x 4096 x 14336: 440 us = 2.19 P op/s, bound by power: the matrix pipes are busy 52 % of the time at 1.86 GHz, where a library
-// product of the same size (2.08 P op/s) has them busy 67 % at 1.43 GHz.  Steps of 64 bytes in four stages: 460 us.
+// 8192 x 4096 x 14336, launches of a trace: 534 us on average, 469 at best = 1.8 and 2.05 P op/s; bound by power: the matrix pipes are
+// busy 52 % of the time at 1.73 GHz, where a library product of the same size (1.94 P op/s) has them busy 66 % at 1.44 GHz.  Steps
+// of 64 bytes in four stages take 4 % longer.
 template <class T, int TN, int TM, int WN, int WM, int S>
 __global__ __launch_bounds__(64 * WN * WM) void gemm_tile(Product p, int tiles_n, int tiles_m) {
     constexpr int BN = 32 * TN * WN, BM = 32 * TM * WM, WAVES = WN * WM, STAGE = (BN + BM) * kRowBytes;
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(64 * WN * WM) void gemm_tile(Product p, int tiles_n
 // Few tokens: bound by reading W once.  A workgroup takes 16 TN channels and 16 TM tokens, K in steps of 256 bytes through a ring
 // of S stages in LDS (whole lines of both operands, S - 1 steps in flight, no registers); of each step its four waves take 64 bytes
 // each (v_mfma_i32_16x16x64_i8), and their integer sums meet in LDS.  Piece c of row r lies at place c ^ r.  Straight from memory
-// into registers -- 16 rows' half lines an instruction -- 45 MB of W took 20.9 us at 32 tokens, this way 13.5.
+// into registers -- 16 rows' half lines an instruction -- 45 MB of W took 20.9 us at 32 tokens, this way 13.6 on average and 12.1 at best.
 constexpr int kFewWaves = 4;
 
 template <class T, int TN, int TM, int S>
@@ -544,11 +545,12 @@ int launch(const Product &p, hipStream_t st) {
     if (p.M <= 32) return wide ? launch_few<T, 2, 2, 4>(p, st) : launch_few<T, 1, 2, 5>(p, st);
     if (p.M <= 64 && !wide) return launch_few<T, 1, 4, 4>(p, st);
     auto tiles = [&](int bn, int bm) { return (p.N + bn - 1) / bn * ((p.M + bm - 1) / bm); };
-    // Larger tiles read less, smaller ones fill the chip and keep more steps in flight.  Measured (us, with the quantisation; the four
-    // tiles in the order below):   4400 x 256 x 2048     18    18    24    32
-    //                              1000 x 4096 x 4096    62    41    43    56
-    //                              512 x 4096 x 4096     60    38    26    32
-    //                              100 x 4096 x 4096     56    36    21    17
+    // Larger tiles read less, smaller ones fill the chip and keep more steps in flight.  Measured (bf16, us, with the quantisation; the
+    // four tiles in the order below):   4400 x 256 x 2048     18    17    23    20
+    //                                   1000 x 4096 x 4096    58    32    37    36
+    //                                   512 x 4096 x 4096     56    29    22    22
+    //                                   100 x 4096 x 4096     52    26    19    15
+    //                                   8192 x 4096 x 14336   465   552   798   769
     if (tiles(256, 256) >= 256) return launch_tile<T, 4, 2, 2, 4, 2>(p, st);
     if (tiles(128, 128) >= 224) return launch_tile<T, 2, 2, 2, 2, 2>(p, st);
     if (tiles(128, 64) >= 128) return launch_tile<T, 2, 1, 2, 2, 4>(p, st);

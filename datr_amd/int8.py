@@ -47,7 +47,7 @@ def _quantize(x2: torch.Tensor):
 def quantize_rows(x: torch.Tensor):
     """x [..., K] -> (q int8 [..., K], scale float32 [...]) with x ~ q * scale[..., None]: scale = max|x| / 127 over the row; x is
     taken as a constant.  A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN (and q 0).  q's rows are held
-    at a distance of whole 128-byte lines, the layout that `linear_int8` reads without a copy."""
+    at a distance of a multiple of 256 bytes, the layout that `linear_int8` reads without a copy."""
     _check_float(x, "quantize_rows")
     if not x.is_cuda:
         raise RuntimeError("quantize_rows: Not implemented on the CPU")
