@@ -112,7 +112,8 @@ __device__ __forceinline__ void finish(bool live, int64_t r, int x, const T *row
     t = join_row<G>(t, c, lds);
     float sum = 0.f;
     if (live && kept_any(t.m, t.s)) {
-        // tau once into the logits' differences and once more into the sum: tau^2 and quotients by tau leave fp32 long before the loss does
+        // tau goes once into the logarithms beside the logits' differences and once into the sum: tau^2 and quotients by tau leave fp32
+        // long before the loss does
         const float log_s = tau * logf(a.s), log_t = tau * logf(t.s);
         for (int j = x; j < sl.k; j += G) {
             const int64_t i = sl.index[r * sl.k + j];

@@ -6,8 +6,8 @@
 // The integer sum is exact (|sum| <= 127 * 128 * K < 2^31 for K <= 131072), so y does not depend on tiles or on the order of sums.
 //
 // Two launches (one for a single token): the rows of x are quantised (bound by memory: x once, q once; 88 892 x 2048 fp32: 147 us on
-// average, 136 at best = 6.2 and 6.7 TB/s), then multiplied.  The product's W is the matrix instruction's first operand: a lane then holds four consecutive
-// channels of one token, which leave as one 8- or 16-byte piece.
+// average, 136 at best = 6.2 and 6.7 TB/s), then multiplied.  The product's W is the matrix instruction's first operand: a lane then
+// holds four consecutive channels of one token, which leave as one 8- or 16-byte piece.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
